@@ -15,7 +15,6 @@ each with the gradients that the optimizer's buckets then carry:
 `own` chooses the side: False computes the formulas with elementary torch operations in 32 bits
 (64 for the table gradient's sums, which may run over thousands of rows), True calls esgd.ops.
 """
-import functools
 import math
 import os
 import sys
@@ -28,8 +27,7 @@ DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 BYTES = {"f32": 4, "bf16": 2, "f16": 2}
 
 
-@functools.lru_cache(maxsize=1)
-def _ops():   # once, as a program imports it
+def _ops():
     here = os.path.join(os.getcwd(), "eager-sgd_amd")
     if here not in sys.path:
         sys.path.insert(0, here)
