@@ -101,6 +101,18 @@ Tensor rows_of(const Tensor &t, int64_t width) {
     return r.stride(1) != 1 && width > 1 ? r.contiguous() : r;
 }
 
+// Whether `out`, contiguous, lies among the elements of `rows` (rows_of's): addresses are compared, row
+// by row, since torch's own question (get_overlap_status) has no answer where rows stand apart.
+bool touches(const Tensor &rows, const Tensor &out) {
+    if (!rows.numel() || !out.numel()) return false;
+    const auto at = [](const Tensor &t) { return reinterpret_cast<intptr_t>(t.const_data_ptr()); };
+    const int64_t size = rows.element_size(), row = rows.size(1) * size, pitch = rows.stride(0) * size;
+    const int64_t from = at(out) - at(rows), to = from + int64_t(out.nbytes());   // of out, from the first row
+    // the first row that ends behind `from`
+    const int64_t i = from < row || !pitch ? 0 : (from - row) / pitch + 1;
+    return i < rows.size(0) && i * pitch < to && i * pitch + row > from;
+}
+
 void check(int rc, const char *what) {
     if (C10_UNLIKELY(rc)) py::module_::import("esgd._lib").attr("check")(rc, what);   // raises EsgdError
 }
@@ -172,8 +184,12 @@ Tensor embedding_grad(const Tensor &grad, const Tensor &tokens, int64_t num_rows
            " rows give a gradient of that type or float32, not ", name_of(table_type));
     size_t bytes = 0;
     check(c.esgd_embedding_grad_work(tokens.numel(), num_rows, width, &bytes), "esgd_embedding_grad_work");
-    on_device(who, grad, {&tokens, &out});
     const Tensor g = rows_of(grad, width), t = tokens.contiguous();
+    if (out.defined()) {
+        REFUSE(touches(g, out), who, ": out shares memory with grad");
+        REFUSE(touches(t.view({1, t.numel()}), out), who, ": out shares memory with tokens");
+    }
+    on_device(who, grad, {&tokens, &out});
     Tensor table = out.defined() ? out : at::empty({num_rows, width}, grad.options().dtype(table_type));
     const Tensor work = work_of(grad, bytes);
     call("esgd_embedding_grad", g, [&](void *s) {

@@ -167,3 +167,22 @@ def test_embedding_grad_refuses_an_out_that_shares_memory():
     _refuses("shares memory with tokens", ops.embedding_grad, torch.zeros(5, 4), t, 2,
              out=t.view(torch.float32)[:8].view(2, 4))
     _refuses("no CPU path", ops.embedding_grad, buf[:20].view(5, 4), t, 5, out=buf[20:].view(5, 4))
+
+
+def test_embedding_grad_refuses_an_out_among_the_rows_it_reads():
+    # rows that stand apart are read where they lie: the table's zeros must not go there
+    buf, t = torch.zeros(10, 8), torch.zeros(10, dtype=torch.long)
+    flat = buf.view(-1)
+    _refuses("shares memory with grad", ops.embedding_grad, buf[:, :4], t, 10, out=flat[:40].view(10, 4))
+    _refuses("shares memory with grad", ops.embedding_grad, buf[:, :4], t, 1, out=flat[75:79].view(1, 4))
+    _refuses("shares memory with grad", ops.embedding_grad, buf[::2], t[:5], 5, out=buf[:5])
+    _refuses("shares memory with grad", ops.embedding_grad, buf[0].expand(10, 8), t, 10, out=buf)
+    _refuses("shares memory with grad", ops.embedding_grad, buf[:, None, 2:5], t[:, None], 2, out=flat[1:7].view(2, 3))
+    # a copy of the caller's that names the same memory in a storage of its own
+    alias = torch.frombuffer(memoryview(buf.numpy()).cast("B"), dtype=torch.float32)
+    _refuses("shares memory with grad", ops.embedding_grad, buf[:, :4], t, 10, out=alias[:40].view(10, 4))
+    # between the rows, behind them and in memory of its own: sound
+    for rows, out in ((1, flat[4:8].view(1, 4)), (1, flat[76:80].view(1, 4)), (2, torch.zeros(2, 4)), (0, flat[:0].view(0, 4))):
+        _refuses("no CPU path", ops.embedding_grad, buf[:, :4], t, rows, out=out)
+    # what is copied before the table is zeroed
+    _refuses("no CPU path", ops.embedding_grad, buf[:, ::2], t, 10, out=flat[:40].view(10, 4))
