@@ -10,7 +10,9 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cstdint>
@@ -74,10 +76,17 @@ std::string shape_of(at::IntArrayRef s) {
         if (C10_UNLIKELY(cond)) throw py::value_error(c10::str(__VA_ARGS__)); \
     } while (0)
 
+// Forward-mode derivatives stop here: a result without its tangent would tell of a derivative of zero.
+// (In an autograd function's forward pass tangents are hidden until the mode is on again.)
+void no_tangent(const char *who, const char *name, const Tensor &t) {
+    const c10::AutoFwGradMode seen(true);
+    REFUSE(t._fw_grad(0).defined(), who, ": ", name, " has a tangent; there is no forward-mode derivative");
+}
 int float_of(const char *who, const char *name, const Tensor &t, int64_t dims = -1) {
     const int code = type_of(t.scalar_type());
     REFUSE(!code, who, ": ", name, " is ", name_of(t.scalar_type()), "; float32, bfloat16 or float16 is needed");
     REFUSE(t.is_neg(), who, ": ", name, " is a view whose sign is still to be changed; resolve_neg() makes it a tensor");
+    no_tangent(who, name, t);
     REFUSE(dims >= 0 && t.dim() != dims, who, ": ", name, " has ", t.dim(), " dimensions, not ", dims);
     return code;
 }
@@ -169,6 +178,7 @@ Tensor embedding_grad(const Tensor &grad, const Tensor &tokens, int64_t num_rows
     REFUSE(num_rows < 0, who, ": num_rows ", num_rows, " is negative");
     REFUSE(accumulate && !out.defined(), who, ": accumulate needs out");
     if (out.defined()) {
+        no_tangent(who, "out", out);
         REFUSE(out.dim() != 2 || out.size(0) != num_rows || out.size(1) != width || !out.is_contiguous(), who,
                ": out is not a contiguous (", num_rows, ", ", width, ") tensor");
         for (const Tensor *t : {&grad, &tokens}) {

@@ -5,11 +5,12 @@ each with its gradient (C ABI: include/esgd_ops.h, which has the formulas).
 They take torch tensors on a HIP device and run on the caller's current stream of that device;
 nothing waits for the GPU, so all of them can be captured into a graph.  embedding,
 expert_dispatch, expert_combine and distill_loss take part in autograd (once; their gradients
-have no gradients); the *_grad functions are the same gradients called directly, for training
-steps that keep their own buckets -- embedding_grad can add into the one that the optimizer
-reduces.  float32, bfloat16 and float16; sums are fp32, in a fixed order, so the same call gives
-the same bits on every replica.  Inputs whose rows are contiguous are read where they lie, at any
-distance and alignment; others are copied first.  There is no CPU path.
+have no gradients, and a tensor with a forward-mode tangent is refused); the *_grad functions are
+the same gradients called directly, for training steps that keep their own buckets --
+embedding_grad can add into the one that the optimizer reduces.  float32, bfloat16 and float16;
+sums are fp32, in a fixed order, so the same call gives the same bits on every replica.  Inputs
+whose rows are contiguous are read where they lie, at any distance and alignment; others are
+copied first.  There is no CPU path.
 """
 from __future__ import annotations
 

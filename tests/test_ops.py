@@ -4,6 +4,7 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from esgd import _lib, ops
 
@@ -186,3 +187,38 @@ def test_embedding_grad_refuses_an_out_among_the_rows_it_reads():
         _refuses("no CPU path", ops.embedding_grad, buf[:, :4], t, rows, out=out)
     # what is copied before the table is zeroed
     _refuses("no CPU path", ops.embedding_grad, buf[:, ::2], t, 10, out=flat[:40].view(10, 4))
+
+
+def _every_call():
+    """Each operator on small tensors that it accepts but for their device, as (operator, its
+    arguments, the places of the floating tensors among them)."""
+    w, t = torch.zeros(5, 4), torch.zeros(3, dtype=torch.long)
+    order = ops.ExpertOrder(torch.zeros(5, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32), 4)
+    x, y, k = torch.zeros(3, 4), torch.zeros(6, 4), torch.zeros(3, 2)
+    z, top, i = torch.zeros(2, 7), torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.long)
+    return [(ops.embedding, (w, t), (0,)), (ops.embedding_grad, (x, t, 5), (0,)),
+            (ops.expert_dispatch, (x, order), (0,)), (ops.expert_dispatch_grad, (y, order), (0,)),
+            (ops.expert_combine, (y, k, order), (0, 1)), (ops.expert_combine_grad, (x, y, k, order), (0, 1, 2)),
+            (ops.distill_loss, (z, top, i), (0, 1)), (ops.distill_loss_grad, (z, top, i, torch.ones(2)), (0, 1, 3))]
+
+
+def test_tangents_of_forward_mode_are_refused():
+    # there is no forward-mode derivative: an answer without a tangent would say that it is zero
+    for fn, args, floats in _every_call():
+        _refuses("no CPU path", fn, *args)
+        for at in floats:
+            for wants_grad in (False, True):
+                with forward_ad.dual_level():
+                    primal = args[at].clone().requires_grad_(wants_grad)
+                    dual = forward_ad.make_dual(primal, torch.ones_like(primal))
+                    _refuses("tangent", fn, *args[:at], dual, *args[at + 1:])
+
+            def of_one(x, fn=fn, args=args, at=at):
+                return fn(*args[:at], x, *args[at + 1:])
+
+            with pytest.raises(ValueError, match="tangent"):
+                torch.func.jvp(of_one, (args[at],), (torch.ones_like(args[at]),))
+    out = torch.zeros(5, 4)
+    with forward_ad.dual_level():
+        _refuses("tangent", ops.embedding_grad, torch.zeros(3, 4), torch.zeros(3, dtype=torch.long), 5,
+                 out=forward_ad.make_dual(out, out))
