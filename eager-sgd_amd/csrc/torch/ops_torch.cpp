@@ -82,10 +82,13 @@ void no_tangent(const char *who, const char *name, const Tensor &t) {
     const c10::AutoFwGradMode seen(true);
     REFUSE(t._fw_grad(0).defined(), who, ": ", name, " has a tangent; there is no forward-mode derivative");
 }
+void no_sign(const char *who, const char *name, const Tensor &t) {
+    REFUSE(t.is_neg(), who, ": ", name, " is a view whose sign is still to be changed; resolve_neg() makes it a tensor");
+}
 int float_of(const char *who, const char *name, const Tensor &t, int64_t dims = -1) {
     const int code = type_of(t.scalar_type());
     REFUSE(!code, who, ": ", name, " is ", name_of(t.scalar_type()), "; float32, bfloat16 or float16 is needed");
-    REFUSE(t.is_neg(), who, ": ", name, " is a view whose sign is still to be changed; resolve_neg() makes it a tensor");
+    no_sign(who, name, t);
     no_tangent(who, name, t);
     REFUSE(dims >= 0 && t.dim() != dims, who, ": ", name, " has ", t.dim(), " dimensions, not ", dims);
     return code;
@@ -178,6 +181,7 @@ Tensor embedding_grad(const Tensor &grad, const Tensor &tokens, int64_t num_rows
     REFUSE(num_rows < 0, who, ": num_rows ", num_rows, " is negative");
     REFUSE(accumulate && !out.defined(), who, ": accumulate needs out");
     if (out.defined()) {
+        no_sign(who, "out", out);
         no_tangent(who, "out", out);
         REFUSE(out.dim() != 2 || out.size(0) != num_rows || out.size(1) != width || !out.is_contiguous(), who,
                ": out is not a contiguous (", num_rows, ", ", width, ") tensor");

@@ -222,3 +222,12 @@ def test_tangents_of_forward_mode_are_refused():
     with forward_ad.dual_level():
         _refuses("tangent", ops.embedding_grad, torch.zeros(3, 4), torch.zeros(3, dtype=torch.long), 5,
                  out=forward_ad.make_dual(out, out))
+
+
+def test_embedding_grad_refuses_an_out_with_a_sign_to_come():
+    # a negated view is contiguous, but its memory is read with the other sign
+    g, t = torch.zeros(3, 4), torch.zeros(3, dtype=torch.long)
+    out = torch._neg_view(torch.ones(5, 4))
+    assert out.is_contiguous() and out.is_neg()
+    for accumulate in (False, True):
+        _refuses("resolve_neg", ops.embedding_grad, g, t, 5, out=out, accumulate=accumulate)
