@@ -183,6 +183,8 @@ Tensor embedding_grad(const Tensor &grad, const Tensor &tokens, int64_t num_rows
     if (out.defined()) {
         no_sign(who, "out", out);
         no_tangent(who, "out", out);
+        REFUSE(out.requires_grad() && c10::GradMode::is_enabled(), who,
+               ": out requires a gradient, and autograd does not see what is written to it (torch.no_grad() or detach())");
         REFUSE(out.dim() != 2 || out.size(0) != num_rows || out.size(1) != width || !out.is_contiguous(), who,
                ": out is not a contiguous (", num_rows, ", ", width, ") tensor");
         for (const Tensor *t : {&grad, &tokens}) {

@@ -231,3 +231,14 @@ def test_embedding_grad_refuses_an_out_with_a_sign_to_come():
     assert out.is_contiguous() and out.is_neg()
     for accumulate in (False, True):
         _refuses("resolve_neg", ops.embedding_grad, g, t, 5, out=out, accumulate=accumulate)
+
+
+def test_embedding_grad_refuses_an_out_that_requires_a_gradient():
+    # as torch's own calls with out=: autograd would not know of the write
+    g, t = torch.zeros(3, 4), torch.zeros(3, dtype=torch.long)
+    leaf = torch.ones(5, 4, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        for accumulate in (False, True):
+            _refuses("requires a gradient", ops.embedding_grad, g, t, 5, out=out, accumulate=accumulate)
+            with torch.no_grad():
+                _refuses("no CPU path", ops.embedding_grad, g, t, 5, out=out, accumulate=accumulate)
