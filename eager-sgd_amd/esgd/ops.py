@@ -70,12 +70,20 @@ def _load():
 _ops = _load()
 
 
+def _number(who: str, name: str, x):
+    """Refuses a tensor where a number is taken: its gradient would be lost, and the call would
+    wait for the GPU to read it."""
+    if isinstance(x, torch.Tensor):
+        raise ValueError(f"{who}: {name} is a tensor; a number is needed (no gradient goes there)")
+
+
 # ---- embedding -----------------------------------------------------------------------------
 
 def _padding(who: str, padding_index) -> int:
     """The row without gradient as the C calls take it, -1 for none."""
     if padding_index is None:
         return -1
+    _number(who, "padding_index", padding_index)
     if padding_index < 0:
         raise ValueError(f"{who}: padding_index {padding_index} is negative (tokens outside the table need none)")
     return int(padding_index)
@@ -88,6 +96,8 @@ def embedding_grad(grad, tokens, num_rows: int, scale: float = 1.0, *, padding_i
     padding_index give nothing.  dtype: grad's own (default) or float32.  out: a contiguous
     tensor to write (its dtype counts then); accumulate=True adds to it instead, and reads and
     writes only the rows that the tokens name."""
+    _number("embedding_grad", "num_rows", num_rows)
+    _number("embedding_grad", "scale", scale)
     return _ops.embedding_grad(grad, tokens, num_rows, scale, _padding("embedding_grad", padding_index), dtype, out,
                                accumulate)
 
@@ -113,6 +123,7 @@ def embedding(weight, tokens, scale: float = 1.0, *, padding_index: int | None =
     padding, say -1 -- reads as zeros and gives no gradient; padding_index is a row that is read
     as it is but gets no gradient either.  dtype: the result's, weight's own by default; a
     float32 table also gives bfloat16 or float16 rows.  The gradient is dense, of weight's dtype."""
+    _number("embedding", "scale", scale)
     if padding_index is not None:
         _padding("embedding", padding_index)
     if weight.requires_grad and torch.is_grad_enabled():
@@ -148,6 +159,7 @@ def expert_sort(experts, num_experts: int) -> ExpertOrder:
     """The order of the pairs of `experts` ((tokens, choices) or (tokens,), int32 or int64) by
     expert, equal experts by (token, choice).  Pairs whose expert is outside [0, num_experts)
     are dropped: they come last and take no part in dispatch and combine."""
+    _number("expert_sort", "num_experts", num_experts)
     offsets, slots = _ops.expert_sort(experts, num_experts)
     return ExpertOrder(offsets, slots, num_experts)
 
@@ -231,6 +243,7 @@ def distill_loss(logits, top_logits, top_index, temperature: float = 1.0):
     order, the teacher a constant.  Entries outside the vocabulary (-1: none) and those of -inf
     take no part; an index that stands there twice counts twice.  A row left without any entry has
     loss and gradient 0 whatever its logits are.  logits of -inf have no share."""
+    _number("distill_loss", "temperature", temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         return _Distill.apply(logits, top_logits, top_index, temperature)
     return _ops.distill_loss(logits, top_logits, top_index, temperature)[0]
@@ -240,4 +253,5 @@ def distill_loss_grad(logits, top_logits, top_index, row_grad, temperature: floa
     """(loss, grad_logits) of distill_loss at once, where the losses' gradients are known before:
     grad_logits = row_grad[r] * d loss[r] / d logits, contiguous, in logits' dtype.  row_grad: float32,
     of the loss's shape (1 / rows for the mean; an expanded scalar will do)."""
+    _number("distill_loss_grad", "temperature", temperature)
     return _ops.distill_loss_grad(logits, top_logits, top_index, row_grad, temperature)

@@ -2,6 +2,7 @@
 The operators' results are in test_ops_gpu.py."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -242,3 +243,24 @@ def test_embedding_grad_refuses_an_out_that_requires_a_gradient():
             _refuses("requires a gradient", ops.embedding_grad, g, t, 5, out=out, accumulate=accumulate)
             with torch.no_grad():
                 _refuses("no CPU path", ops.embedding_grad, g, t, 5, out=out, accumulate=accumulate)
+
+
+def test_tensors_in_the_place_of_numbers_are_refused():
+    # their gradient would be lost, and on a GPU the call would wait for their value
+    w, t, e = torch.zeros(5, 4), torch.zeros(3, dtype=torch.long), torch.zeros(3, 2, dtype=torch.int32)
+    z, top, i = torch.zeros(2, 7), torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.long)
+    for x in (torch.tensor(2.0), torch.tensor(2.0, requires_grad=True), torch.nn.Parameter(torch.ones(1))):
+        for weight in (w, torch.zeros(5, 4, requires_grad=True)):
+            _refuses("scale is a tensor", ops.embedding, weight, t, x)
+        _refuses("scale is a tensor", ops.embedding_grad, torch.zeros(3, 4), t, 5, x)
+        for logits in (z, torch.zeros(2, 7, requires_grad=True)):
+            _refuses("temperature is a tensor", ops.distill_loss, logits, top, i, x)
+        _refuses("temperature is a tensor", ops.distill_loss_grad, z, top, i, torch.ones(2), x)
+    one = torch.tensor(1)
+    _refuses("padding_index is a tensor", ops.embedding, w, t, padding_index=one)
+    _refuses("padding_index is a tensor", ops.embedding_grad, torch.zeros(3, 4), t, 5, padding_index=one)
+    _refuses("num_rows is a tensor", ops.embedding_grad, torch.zeros(3, 4), t, one)
+    _refuses("num_experts is a tensor", ops.expert_sort, e, one)
+    for number in (2, 2.0, True, np.float32(2.0), np.int64(2)):   # any other number will do
+        _refuses("no CPU path", ops.embedding, w, t, number)
+        _refuses("no CPU path", ops.distill_loss, z, top, i, number)
