@@ -214,8 +214,16 @@ int rows_per_tile(int64_t n, int64_t chunks, int lane_bytes) {
     while (per > 8 && (n + per - 1) / per * chunks * lane_bytes < 2048 * 16) per /= 2;
     return per;
 }
-size_t part_bytes(int64_t n, int64_t width) {   // with the smallest tile
-    return size_t((n + 7) / 8) * 2 * size_t(width) * 4;
+template <class G, class W>
+int rows_per_tile_of(int64_t n, int64_t width) {
+    constexpr int E = sum_elems<W>;
+    return rows_per_tile(n, (width + 64 * E - 1) / (64 * E), E * int(sizeof(G)));
+}
+// two rows a tile, with the shortest tiles that any of the types have
+size_t part_bytes(int64_t n, int64_t width) {
+    const int64_t per = std::min({rows_per_tile_of<f32_t, f32_t>(n, width), rows_per_tile_of<bf16_t, f32_t>(n, width),
+                                  rows_per_tile_of<bf16_t, bf16_t>(n, width)});
+    return size_t((n + per - 1) / per) * 2 * size_t(width) * 4;
 }
 
 template <class W, class O>
@@ -239,7 +247,7 @@ int row_sums(const void *grad, int64_t grad_pitch, int64_t n, int64_t width, con
              hipStream_t s) {
     constexpr int E = sum_elems<W>;
     const int64_t chunks = (width + 64 * E - 1) / (64 * E);
-    const int per = rows_per_tile(n, chunks, E * int(sizeof(G)));
+    const int per = rows_per_tile_of<G, W>(n, width);
     const int64_t tiles = (n + per - 1) / per, items = tiles * chunks;
     hipLaunchKernelGGL((k_row_sums<G, W>), dim3(unsigned((items + 3) / 4)), dim3(256), 0, s,
                        static_cast<const G *>(grad), grad_pitch, n, width, key, place, uint32_t(rows), per, scale,

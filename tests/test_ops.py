@@ -264,3 +264,30 @@ def test_tensors_in_the_place_of_numbers_are_refused():
     for number in (2, 2.0, True, np.float32(2.0), np.int64(2)):   # any other number will do
         _refuses("no CPU path", ops.embedding, w, t, number)
         _refuses("no CPU path", ops.distill_loss, z, top, i, number)
+
+
+def test_embedding_grad_asks_for_the_work_memory_that_it_uses():
+    # the sort's share, which a width of 0 shows alone, and two fp32 rows for every tile of sorted
+    # rows.  Tiles are 64 rows, halved down to 8 until their loads -- lane_bytes for each 64 * columns
+    # of a tile -- are 2048 waves' of 16 bytes; (columns, lane_bytes) of the gradient's and table's types:
+    types = {(F, F): (4, 16), (BF, F): (4, 8), (BF, BF): (8, 16)}
+    h, z = _lib.lib(), C.c_size_t()
+
+    def asked(n, width):
+        assert h.esgd_embedding_grad_work(n, 1000, width, C.byref(z)) == 0
+        return z.value
+
+    def tiles(n, width, columns, lane_bytes):
+        chunks, per = -(-width // (64 * columns)), 64
+        while per > 8 and -(-n // per) * chunks * lane_bytes < 2048 * 16:
+            per //= 2
+        return -(-n // per)
+
+    sizes = [(n, w) for n in (1, 7, 8, 9, 4095, 4096, 32767, 32768, 65536, 65537, 131072, 262144, 1048576)
+             for w in (1, 255, 256, 257, 512, 513, 1000, 1024, 4096)]
+    for n in (8192, 16384, 16385, 32768, 32769):   # both sides of every change of the tile's rows
+        sizes += [(n * k + d, w) for k in (1, 2, 4) for d in (-1, 0, 1) for w in (256, 512, 1024)]
+    for n, w in sizes:
+        most = max(tiles(n, w, *t) for t in types.values())
+        assert asked(n, w) - asked(n, 0) == most * 2 * w * 4, (n, w)
+    assert asked(131072, 1024) < 20 << 20   # 130 MiB with room for tiles of 8

@@ -9,12 +9,13 @@ result type's half step (2^-24, bf16 2^-8, fp16 2^-11, with half its smallest su
     (4 T + 2) u with T the row's largest |d| / temperature; the sum of V shares adds V' u with V'
     the longest chain of additions and rescalings, at most V / 64 + 128 in any of the kernels
 """
+import ctypes as C
 import math
 
 import pytest
 import torch
 
-from esgd import ops
+from esgd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -948,3 +949,24 @@ def test_distill_gradient_of_very_many_rows():
     got = grad_of(*(x.repeat(times, 1)[:n] for x in (z, t, index)))
     assert torch.equal(got[:n // few * few].view(-1, few, v), want.expand(n // few, few, v))
     assert torch.equal(got[n // few * few:], want[:n % few])
+
+
+@pytest.mark.parametrize("gdt,wdt", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("n,d", [(1, 5), (4095, 1000), (4096, 512), (16384, 256), (16385, 257), (32769, 1024), (65536, 513), (65537, 512)])
+def test_embedding_grad_stays_in_its_work_memory(gdt, wdt, n, d):
+    # exactly what it asks for, with marked bytes behind; half the rows are one token's, so that
+    # every tile leaves partial sums
+    h, size, v = _lib.lib(), C.c_size_t(), 301
+    _lib.check(h.esgd_embedding_grad_work(n, v, d, C.byref(size)))
+    work = torch.full((size.value + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+    g = gen(n + d)
+    grad, out = normal(g, n, d, dtype=gdt), torch.empty(v, d, dtype=wdt, device=DEV)
+    t = torch.randint(0, v, (n,), device=DEV, generator=g)
+    t[::2] = 7
+    code = {F32: _lib.FLOAT, BF16: _lib.BF16, F16: ops.HALF}
+    ptr = [C.c_void_p(x.data_ptr()) for x in (grad, t, out, work)]
+    _lib.check(h.esgd_embedding_grad(code[gdt], ptr[0], d, n, d, 64, ptr[1], -1, 0.5, code[wdt], ptr[2], v, 0, ptr[3],
+                                     size.value, C.c_void_p(torch.cuda.current_stream().cuda_stream or 1)))
+    assert (work[size.value:] == 0xA5).all()
+    want, bound = grad_want(grad, t, v, 0.5)
+    close(out, want, rounded(want, wdt, bound))
