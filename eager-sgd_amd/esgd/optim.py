@@ -192,7 +192,9 @@ class EagerSGDOptimizer:
                 raise RuntimeError("EagerSGDOptimizer(fuse=True, overlap=True): a parameter of a bucket has no "
                                    "gradient, but the bucket's schedule is persistent")
             if g.is_sparse:
-                return False   # apply_gradients makes it dense first
+                if made is None:
+                    return False   # apply_gradients makes it dense
+                g = _dense(g, p, made)
             if g.dtype != torch.float32 or not g.is_contiguous():
                 if made is None:
                     return False   # apply_gradients posts it

@@ -73,3 +73,35 @@ def test_registered_torch_op_sits_in_traced_graphs():
     ar.close()   # unregistered: the operator no longer reaches it
     with pytest.raises(RuntimeError, match="no live op"):
         torch.ops.esgd.allreducef(torch.ones(4, 3), torch.ones(4, 3), handle, 2.0)
+
+
+def test_bucket_with_a_sparse_gradient_outside_the_list_is_still_reduced(monkeypatch):
+    # fuse=True, overlap=True reduces whole buckets of p.grad, whatever part of them the caller
+    # hands to apply_gradients: a sparse gradient among the others is made dense, not left out
+    import torch
+    posted = []
+
+    class Op:
+        def __init__(self, shape):
+            self.count = shape[0]
+
+        def post_packed(self, srcs, dsts, divisor, stream):
+            posted.append([g.clone() for g in srcs])
+            assert sum(g.numel() for g in srcs) == self.count and not any(g.is_sparse for g in srcs)
+
+        def wait_packed(self, stream):
+            pass
+
+    monkeypatch.setattr(deep500, "AllreduceOp", Op)
+    monkeypatch.setattr(deep500, "configure", lambda *a: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: type("S", (), {"cuda_stream": 0}))
+    emb, head = torch.nn.Embedding(11, 4, sparse=True), torch.nn.Linear(4, 3)
+    opt = EagerSGDOptimizer(torch.optim.SGD([*emb.parameters(), *head.parameters()], lr=0.1), 2, mode="allreduce",
+                            fuse=True, overlap=True)
+    head(emb(torch.tensor([1, 5, 5])).sum(0)).sum().backward()
+    want = emb.weight.grad.to_dense()
+    assert emb.weight.grad.is_sparse and not posted   # no post from the hooks: the bucket waits
+    opt._reduce([(p.grad, p) for p in head.parameters()], 0)
+    assert len(posted) == 1 and not emb.weight.grad.is_sparse
+    assert any(g.shape == want.shape and torch.equal(g, want) for g in posted[0])
+    opt.detach()
