@@ -6,13 +6,12 @@
 //
 // Gradient: sum of the output's gradient rows by token.  The tokens are sorted first
 // (row_sort.hip), so equal tokens lie together and every sum has one order; float atomics would
-// need none of that but give other bits at every call, and replicas that are to stay identical
-// cannot have them.  The sorted rows are cut into tiles of equal length, whatever
+// need none of that but give other bits at every call, and no run could be repeated.  The sorted rows are cut into tiles of equal length, whatever
 // the tokens: a wave walks its tile's rows for 64 x 16 bytes of columns, adding in registers,
 // and stores a table row where a token's run ends.  A run that crosses tiles leaves fp32
 // partial sums, which k_row_join adds up in the order of the tiles; a token that half the
-// batch consists of is thus spread over the chip like any other.  The table's other rows are
-// zeroed while the sort runs.
+// batch consists of is thus spread over the chip like any other.  The whole table is zeroed while
+// the sort runs; rows with a token are written a second time.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

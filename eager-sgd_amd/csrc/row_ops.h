@@ -28,10 +28,11 @@ template <class T, int N>
 __device__ __forceinline__ vec<T, N> load_vec(const T *p) {
     return *reinterpret_cast<const vec<T, N> *>(p);
 }
-// Stores stream past the caches (nontemporal): what is written here is larger than they are
-// or is read by another kernel later, and lines that wait there to be written back hold up the
-// next kernel's reads (16384 x 8 rows of 2048 bf16, out and back with gradients: 612 us of kernels
-// with plain stores, 560 with these, though the way out alone takes 116 instead of 101).
+// Stores stream past the caches (nontemporal): the largest results do not fit there, and lines
+// that wait to be written back hold up the next kernel's reads (16384 x 8 rows of 2048 bf16, out
+// and back with gradients: 612 us of kernels with plain stores, 560 with these, though the way out
+// alone takes 116 instead of 101).  Measured with these kernels one after the other; with a
+// product that reads a few MB of rows in between it has not been.
 template <class T, int N>
 __device__ __forceinline__ void store_vec(T *p, vec<T, N> v) {
     __builtin_nontemporal_store(v, reinterpret_cast<vec<T, N> *>(p));

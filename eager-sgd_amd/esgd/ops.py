@@ -8,7 +8,7 @@ expert_dispatch, expert_combine and distill_loss take part in autograd (once; th
 have no gradients, and a tensor with a forward-mode tangent is refused); the *_grad functions are
 the same gradients called directly, for training steps that keep their own buckets --
 embedding_grad can add into the one that the optimizer reduces.  float32, bfloat16 and float16;
-sums are fp32, in a fixed order, so the same call gives the same bits on every replica.  Inputs
+sums are fp32, in a fixed order, so the same call gives the same bits every time.  Inputs
 whose rows are contiguous are read where they lie, at any distance and alignment; others are
 copied first.  There is no CPU path.
 """

@@ -63,7 +63,7 @@ def _dense(grad, param, made):
     """The dense fp32 gradient of an embedding's sparse one (nn.Embedding(sparse=True)), put in
     param.grad: TF 1.x makes its IndexedSlices dense in the same place, on the way into the
     reference's op (opt_esgd_solo_imagenet_imbalance.py:40).  The rows of a token are summed in
-    their order by one kernel (ops.embedding_grad), not by atomics: replicas stay identical."""
+    their order (ops.embedding_grad), not by atomics: the same tokens and values give the same bits."""
     if grad is None or not grad.is_sparse:
         return grad
     import torch

@@ -67,11 +67,13 @@ int esgd_expert_dispatch_grad(int type, const void *grad_rows, int64_t grad_pitc
                               int64_t choices, int64_t width, const int32_t *slots, void *grad_x,
                               void *stream);
 /* out[t] = sum over j of weights[t, j] * rows[slot(t, j)], in the order of j.  weights: fp32,
- * contiguous; those of dropped pairs are not read. */
+ * contiguous.  The weights of dropped pairs and the rows at their places change nothing, whatever
+ * they are, but have to be memory that can be read. */
 int esgd_expert_combine(int type, const void *rows, int64_t rows_pitch, int64_t tokens, int64_t choices,
                         int64_t width, const int32_t *slots, const float *weights, void *out, void *stream);
 /* grad_rows[slot(t, j)] = weights[t, j] * grad[t] (zeros for dropped pairs; wholly written) and
- * grad_weights[t, j] = <grad[t], rows[slot(t, j)]> (0 for dropped pairs) */
+ * grad_weights[t, j] = <grad[t], rows[slot(t, j)]> (0 for dropped pairs; what stands
+ * in their weights and rows changes nothing, but has to be memory that can be read) */
 int esgd_expert_combine_grad(int type, const void *grad, int64_t grad_pitch, const void *rows,
                              int64_t rows_pitch, int64_t tokens, int64_t choices, int64_t width,
                              const int32_t *slots, const float *weights, void *grad_rows,
@@ -82,7 +84,8 @@ int esgd_expert_combine_grad(int type, const void *grad, int64_t grad_pitch, con
  * [0, vocab), q = softmax(logits / temperature) over the whole row,
  *   loss = temperature^2 * sum_k p_k (log p_k - log q[top_index_k]).
  * An index that stands there twice counts twice.  A row without any entry of finite or +infinite
- * teacher logit has loss 0 and gradient 0, and its logits are not read.
+ * teacher logit has loss 0 and gradient 0, whatever its logits are (they have to be memory that can
+ * be read).
  * stats (4 floats a row): what the gradient needs of the pass. */
 #define ESGD_DISTILL_TOP_MAX 1024
 int esgd_distill_work(int64_t n, int64_t vocab, size_t *bytes);
