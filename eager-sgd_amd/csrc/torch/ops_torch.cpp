@@ -2,7 +2,7 @@
 //
 // Checks the tensors, allocates the results and work memory (torch's allocator, the current
 // stream) and makes the C calls.  All of a small call's cost is here and in the launch: in Python
-// over ctypes the same steps took 7.6 us for a lookup of 16 tokens, here 4.7, of which the launch is 3.4.
+// over ctypes the same steps took 7.6 us for a lookup of 16 tokens, here 4.5, of which the launch is 3.4.
 // The C entry points come as addresses from esgd._lib, which has loaded libesgd.so, so that there is
 // one library in the process whatever its path.  What a caller got wrong raises ValueError, a
 // failed call EsgdError, as everywhere in the package.
