@@ -970,3 +970,23 @@ def test_embedding_grad_stays_in_its_work_memory(gdt, wdt, n, d):
     assert (work[size.value:] == 0xA5).all()
     want, bound = grad_want(grad, t, v, 0.5)
     close(out, want, rounded(want, wdt, bound))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_embedding_grad_into_the_gap_between_the_rows_it_reads(dtype):
+    # out may lie between rows that stand apart, as close as can be; nothing else is written
+    g = gen(21)
+    n, d, pitch = 300, 12, 100
+    buf = normal(g, n, pitch, dtype=dtype)
+    grad, before = buf[:, 5:5 + d], buf.clone()
+    t = torch.randint(0, 7, (n,), device=DEV, generator=g)
+    want, bound = grad_want(grad, t, 7, 0.5)
+    start = 17 * pitch + 5 + d
+    out = buf.view(-1)[start:start + 7 * d].view(7, d)   # 84 of the 88 elements between rows 17 and 18
+    ops.embedding_grad(grad, t, 7, 0.5, out=out)
+    close(out, want, rounded(want, dtype, bound))
+    before.view(-1)[start:start + 7 * d] = out.reshape(-1)
+    assert torch.equal(buf, before)
+    for at in (start - 1, start + 5):   # one element into the row before, one into the row behind
+        with pytest.raises(ValueError, match="shares memory with grad"):
+            ops.embedding_grad(grad, t, 7, 0.5, out=buf.view(-1)[at:at + 7 * d].view(7, d))
